@@ -83,7 +83,6 @@ __device__ __forceinline__ float pg_zero(uint32_t word) { return (float)(word & 
 
 template <typename T> struct Pair;            // two values of a 16-bit type in a register
 template <> struct Pair<__half> {
-  static constexpr bool BF16 = false;
   static __device__ __forceinline__ float2 get(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
   static __device__ __forceinline__ uint32_t put(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -92,7 +91,6 @@ template <> struct Pair<__half> {
   static __device__ __forceinline__ __half one(float a) { return __float2half_rn(a); }
 };
 template <> struct Pair<__nv_bfloat16> {
-  static constexpr bool BF16 = true;
   static __device__ __forceinline__ float2 get(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
   static __device__ __forceinline__ uint32_t put(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);

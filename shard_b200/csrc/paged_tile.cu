@@ -18,12 +18,13 @@
 //   warp 12         all products; 13: which values are no numbers (14 and 15 only give their registers away)
 //
 // The eight channels of a 32-bit word are unpacked in the order 0 4 1 5 2 6 3 7, in which two nibbles at a time leave
-// it; queries are staged in that order, and the output is put back.  fp16 outputs have weights in two fp16 parts (22
-// bits), each product run twice; for bf16 outputs, whose own rounding is 8 times a part's, one part is enough.
+// it; queries are staged in that order, and the output is put back.  Weights are two fp16 parts (22 bits, as in
+// paged_attn.cu), each product run twice: the first part alone (bf16 outputs, 415 us) moves one output in twenty by a
+// last place.
 //
-// What bounds it: the chain of a step, 2 690 cycles a job: product with the weights 740, its end 270, scores 1 050, and
-// the softmax of 128 numbers a thread, which the other group's products hide only in part.  2 048 rows x 4 query heads
-// behind 8 192 tokens, 8 KV heads, bf16 (309 GFLOP): 415 us, 745 TFLOP/s; fp16, with the second parts, 675 us.  Start
+// What bounds it: the chain of a step, 4 370 cycles a job: products with the weights, their end, scores, and the
+// softmax of 128 numbers a thread, which the other group's products hide only in part.  2 048 rows x 4 query heads
+// behind 8 192 tokens, 8 KV heads (309 GFLOP): 675 us, 458 TFLOP/s, bf16 and fp16 alike.  Start
 // and result of a piece are some 8 000 cycles each.  Measured and slower: a thread for each group's products (470 us),
 // eight unpacking warps with the scores read from tensor memory twice (485 us).
 #include <atomic>
@@ -235,7 +236,6 @@ __device__ __forceinline__ void fewer_regs() { asm volatile("setmaxnreg.dec.sync
 // ---- the kernel ----------------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_constant__ PagedAttnParams p) {
-  constexpr bool PARTS = sizeof(T) == 2 && !Pair<T>::BF16;   // weights in two parts
   extern __shared__ __align__(128) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* q_s = smem;                             // [group]
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             for (int ks = 0; ks < 8; ++ks) {             // weights of 32 tokens lie in 32 columns, first parts in front
               const uint32_t w = S + 32 * (ks >> 1) + 8 * (ks & 1);
               product_ts(O, w, vd + (uint64_t)((ks * 2048) >> 4), IDESC_O, (j > 1 || ks > 0) ? 1u : 0u);
-              if (PARTS) product_ts(O, w + 16, vd + (uint64_t)((ks * 2048) >> 4), IDESC_O, 1u);
+              product_ts(O, w + 16, vd + (uint64_t)((ks * 2048) >> 4), IDESC_O, 1u);
             }
             commit(O_DONE(g));
             if (!two || g == 1) commit(V_FREE(st));
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
           for (int c = 0; c < 4; ++c) {
             if (c >= c0 && c < c1) continue;
             tmem_st_x16(S + 32 * c, zero);
-            if (PARTS) tmem_st_x16(S + 32 * c + 16, zero);
+            tmem_st_x16(S + 32 * c + 16, zero);
           }
         }
         auto hide = [&](uint32_t (&s)[32], int c) {      // -infinity for what the row does not see of scores 32 c ..
@@ -702,13 +702,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             sum[0] += a;
             sum[1] += d;
             hi[i] = pack_half2(a, d);
-            if (PARTS) {
-              const float2 rest = __half22float2(as_half2(hi[i]));
-              lo[i] = pack_half2(a - rest.x, d - rest.y);
-            }
+            const float2 rest = __half22float2(as_half2(hi[i]));
+            lo[i] = pack_half2(a - rest.x, d - rest.y);
           }
           tmem_st_x16(S + 32 * c, hi);
-          if (PARTS) tmem_st_x16(S + 32 * c + 16, lo);
+          tmem_st_x16(S + 32 * c + 16, lo);
         };
         if (copies == 1) {
           uint32_t s[4][32];
