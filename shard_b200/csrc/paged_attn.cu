@@ -23,6 +23,7 @@
 // sequences of up to 8 192 tokens, 8 KV heads, 4 query heads to each (433 MB): 113 to 117 us, 3.8 TB/s; one of 131 072 (143 MB):
 // 44 us, 3.3 TB/s.  Fixed part of a launch, some 10 000 cycles: adding the list up 2 000, the query 2 000, the first
 // blocks 1 300, joining the warps; then the launch that joins the CTAs, 3 to 5 us.
+#include <atomic>
 #include <type_traits>
 
 #include "paged_attn.cuh"
@@ -611,19 +612,29 @@ static PagedAttnLayout paged_attn_layout(int ratio, int max_new) {
   return l;
 }
 
+static constexpr size_t split_smem(int n_seqs) { return (size_t)PA_WARPS * PA_STAGES * PA_GROUP * PG_BYTES + (size_t)(n_seqs + 1) * 8; }
+
 template <typename T, int COLS>
 static cudaError_t launch_paged_split(const PagedAttnParams& p, int grid, cudaStream_t st) {
-  const size_t smem = (size_t)PA_WARPS * PA_STAGES * PA_GROUP * PG_BYTES + (size_t)(p.c.n_seqs + 1) * 8;
-  cudaError_t e = cudaSuccess;
-  if (smem > 48 * 1024) e = cudaFuncSetAttribute(paged_split_kernel<T, COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // Asked for once on a device, for the most that a call can need: the limit belongs to the kernel, not to the call, and
+  // another thread's call may be between its request and its launch.
+  static std::atomic<bool> configured[MAX_DEVICES];
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= MAX_DEVICES) return cudaErrorInvalidDevice;
+  if (!configured[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(paged_split_kernel<T, COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)split_smem(SHARD_PAGED_MAX_SEQS));
+    if (e != cudaSuccess) return e;
+    configured[dev].store(true, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(32 * PA_WARPS);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = split_smem(p.c.n_seqs);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
