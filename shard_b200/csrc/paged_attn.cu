@@ -34,8 +34,10 @@ constexpr int PA_WARPS = 4;                              // (5, 7, 8: slower)
 constexpr int PA_CTAS = 3;                               // per SM, 168 registers a thread (4 and 128: spills, 135 us where this took 124)
 constexpr int PA_GROUP = 2;                              // blocks that a warp takes at a time (4: no room in registers, slower)
 constexpr int PA_STAGES = 2;                             // such groups in its ring (3: the same)
+constexpr int PA_HOLD = 64;                              // turns of a warp whose products add up in its accumulators (see paged_attn.cuh)
 constexpr int PA_MIN_BLOCKS = 4;                         // of a CTA's run: one for each warp
 constexpr uint32_t PA_NO_BLOCK = 0xffffffffu;
+constexpr int PA_HELD = 32 * 36;                         // numbers in a warp's accumulators, and where they count from
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -437,11 +439,37 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
         }
       }
     };
+    // What the accumulators had before their last PA_HOLD turns waits in memory, with its reference points.
+    float4* held = reinterpret_cast<float4*>(p.part + (int64_t)2 * gridDim.x * COLS * PART + (blockIdx.x * PA_WARPS + warp) * PA_HELD) + lane;
+    const int hold = PA_HOLD * step, first_hold = first + hold;
+    auto add_held = [&]() {
+      const float4 at = held[8 * 32];
+      const float by[2] = {ex2(at.x - ref[0]), ex2(at.y - ref[1])};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 h = held[i * 32];
+        o[i][0] = fmaf(h.x, by[0], o[i][0]);
+        o[i][1] = fmaf(h.y, by[1], o[i][1]);
+        o[i][2] = fmaf(h.z, by[0], o[i][2]);
+        o[i][3] = fmaf(h.w, by[1], o[i][3]);
+      }
+    };
 #pragma unroll 1
-    for (; first < blk1; first += step, slot ^= 1) {
+    for (int next_hold = first_hold; first < blk1; first += step, slot ^= 1) {
+      if (first == next_hold) {
+        if (first != first_hold) add_held();
+        next_hold += hold;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          held[i * 32] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+          o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        }
+        held[8 * 32] = make_float4(lim[0] == PA_MOST_LOG2 ? ref[0] : PA_NOTHING, lim[1] == PA_MOST_LOG2 ? ref[1] : PA_NOTHING, 0.f, 0.f);
+      }
       if (group == PA_GROUP) turn(std::true_type());
       else turn(std::false_type());
     }
+    if (first > first_hold) add_held();
     cp_async_wait<0>();
     __syncwarp();
 
@@ -606,7 +634,7 @@ static PagedAttnLayout paged_attn_layout(int ratio, int max_new) {
   l.grid = (sm_count() > 0 ? sm_count() : 1) * PA_CTAS;
   l.cols = (int64_t)ratio * max_new <= 4 ? 4 : 8;
   l.part = ((size_t)l.grid * sizeof(int4) + 127) & ~(size_t)127;
-  l.tile = (l.part + (size_t)2 * l.grid * l.cols * PART * 4 + 127) & ~(size_t)127;
+  l.tile = (l.part + (size_t)l.grid * (2 * l.cols * PART + PA_WARPS * PA_HELD) * 4 + 127) & ~(size_t)127;
   l.tiles = (int64_t)ratio * max_new > PA_SHORT_ROWS;
   l.bytes = l.tile + (l.tiles ? paged_tile_bytes() : 0);
   return l;

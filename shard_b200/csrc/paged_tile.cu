@@ -44,6 +44,7 @@ constexpr int PT_KEYS = 128;                             // of a tile
 constexpr int PT_TILE_BYTES = 32768;
 constexpr int PT_COL_O = 256;                            // score columns of A, B; accumulators of A, B
 constexpr int PT_BARS = 19;
+constexpr int PT_HOLD = 16;                              // tiles of a group whose products add up in the accumulator (see paged_attn.cuh)
 constexpr int PT_TRIES = 3;                              // lengths of parts that are tried
 constexpr int PT_WALK_BYTES = 128;
 constexpr int PT_SMEM = 1024 + 6 * PT_TILE_BYTES + PT_BARS * 8 + 16 + 256 * 8 + 256 * 4 + 32 + (PT_THREADS + 1) * 8 + (PT_THREADS / 32) * PT_WALK_BYTES + 8;
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {             // weights of 32 tokens lie in 32 columns, first parts in front
               const uint32_t w = S + 32 * (ks >> 1) + 8 * (ks & 1);
-              product_ts(O, w, vd + (uint64_t)((ks * 2048) >> 4), IDESC_O, (j > 1 || ks > 0) ? 1u : 0u);
+              product_ts(O, w, vd + (uint64_t)((ks * 2048) >> 4), IDESC_O, ((j >> 1) % PT_HOLD != 0 || ks > 0) ? 1u : 0u);
               product_ts(O, w + 16, vd + (uint64_t)((ks * 2048) >> 4), IDESC_O, 1u);
             }
             commit(O_DONE(g));
@@ -644,6 +645,25 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
       const int stride = two ? 1 : 2, t_first = walk.k0 + (two ? 0 : g);
       bool missing = t_first < k1 && page_missing(t_first);
       bool fresh = true;                                 // no product in the accumulator yet
+      // (a run has at most two pieces of units that others share: its first piece, and its last)
+      float* records = p.part + (2 * (int64_t)blockIdx.x + (first_piece ? 0 : 1)) * PT_ROWS * PART;
+      // What the accumulator had before its last PT_HOLD tiles waits where the piece's result will go, four channels of
+      // all lanes side by side: held = held * by + accumulator * scale.
+      float held_ref = PA_NOTHING;                       // its reference point
+      float4* held = reinterpret_cast<float4*>(records + (warp * 32) * PART) + lane;
+      auto add_held = [&](uint32_t (&o)[16], int c, float scale, float by, bool has) {   // channels 16 c ..
+        float4 h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = has ? held[(4 * c + i) * 32] : make_float4(0.f, 0.f, 0.f, 0.f);
+        tmem_ld_x16(O + 16 * c, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x[4] = {h[i].x, h[i].y, h[i].z, h[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[4 * i + e] = __float_as_uint(fmaf(x[e], by, __uint_as_float(o[4 * i + e]) * scale));
+        }
+      };
       for (int tile = t_first; tile < k1; tile += stride, ++job) {
         const uint32_t holes = __ballot_sync(0xffffffffu, missing);
         if (tile + stride < k1) missing = page_missing(tile + stride);
@@ -751,7 +771,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         }
         l = l * alpha + (sum[0] + sum[1]);
         // (the group's product before this one has run: the scores were issued behind it)
-        if (!fresh && __any_sync(0xffffffffu, alpha != 1.f)) {
+        const int nth = (tile - t_first) >> (two ? 0 : 1);   // of the group's tiles of the piece
+        if (nth % PT_HOLD == 0 && nth > 0) {             // the product to come begins the accumulator anew
+          const float by = ex2(held_ref - ref);
+#pragma unroll 4
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            add_held(o, c, alpha, by, nth > PT_HOLD);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) held[(4 * c + i) * 32] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                                            __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+          }
+          held_ref = lim == PA_MOST_LOG2 ? ref : PA_NOTHING;
+        } else if (!fresh && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
           for (int c = 0; c < 8; ++c) {
             uint32_t o[16];
@@ -773,8 +805,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
 
       // ---- the piece's result
       const bool finish = walk.whole;
-      // (a run has at most two pieces of units that others share: its first piece, and its last)
-      float* records = p.part + (2 * (int64_t)blockIdx.x + (first_piece ? 0 : 1)) * PT_ROWS * PART;
+      if (k1 - t_first > PT_HOLD * stride && warp_live) {                  // (the records that may lie there are written once all warps have read)
+        const float by = ex2(held_ref - ref);
+#pragma unroll 4
+        for (int c = 0; c < 8; ++c) {
+          uint32_t o[16];
+          add_held(o, c, 1.f, by, true);
+          tmem_st_x16(O + 16 * c, o);
+        }
+        tmem_wait_st();
+        __syncwarp();
+      }
       if (tid == 0 && walk.opens && !finish) {
         int pieces = walk.parts;
         if (pieces == 0) {
