@@ -217,6 +217,22 @@ __device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatil
   *abort_flag = 1;
   return false;
 }
+// The same for what may take as long as a whole piece of work does: the bound counts from the last time that `progress`,
+// which whoever is waited for moves on with every tile, was seen to change.  There is time to sleep here.
+constexpr int PT_LONG_TRIES = 1 << 15;                   // of some 2 microseconds
+__device__ __forceinline__ bool long_wait(uint32_t bar, uint32_t parity, const volatile int* progress, volatile int* abort_flag) {
+  int seen = *progress;
+  for (int i = 0; i < PT_LONG_TRIES; ++i) {
+    if (mbar_try(bar, parity, 1000)) return true;
+    if (*abort_flag) return false;
+    const int now = *progress;
+    if (now != seen) i = 0;
+    seen = now;
+    __nanosleep(1000);
+  }
+  *abort_flag = 1;
+  return false;
+}
 // single-thread forms of the products (the caller is one thread)
 __device__ __forceinline__ void product_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
@@ -248,6 +264,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
   float2* ml_s = reinterpret_cast<float2*>(tmem_slot + 4);         // reference points and sums of rows that several threads have
   float* f_s = reinterpret_cast<float*>(ml_s + 256);               // of a row
   int* tally = reinterpret_cast<int*>(f_s + 256);
+  volatile int* jobs_done = tally + PT_TRIES + 1;                  // moves on with the products,
+  volatile int* looked_at = tally + PT_TRIES + 2;                  // and with the tiles whose values have been looked through
   int64_t* chunks = reinterpret_cast<int64_t*>(tally + 8);        // [threads + 1] steps before each thread's sequences
   int2* odd_s = reinterpret_cast<int2*>(reinterpret_cast<unsigned char*>(chunks + PT_THREADS + 1) + (PT_THREADS / 32) * PT_WALK_BYTES);   // first token of the piece whose values (of each half) are no numbers
   const uint32_t bar0 = smem_u32(bars);
@@ -418,6 +436,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
               product_ts(O, w + 16, vd + (uint64_t)((ks * 2048) >> 4), IDESC_O, 1u);
             }
             commit(O_DONE(g));
+            *jobs_done = (int)(2 * tile0) + j;
             if (!two || g == 1) commit(V_FREE(st));
             // the next scores take the place of the weights
             if (j + 2 < n_jobs) ok = tile_wait(O_DONE(g), job & 1, abort_s);
@@ -457,10 +476,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             first0 = min(first0, first_bad(bad_words(w[i].x), bad_words(w[i].y), at[i]));
             first1 = min(first1, first_bad(bad_words(w[i].z), bad_words(w[i].w), at[i]));
           }
+          if (lane == 0) *looked_at = tile;
         }
         first0 = (int)__reduce_min_sync(0xffffffffu, (uint32_t)first0);
         first1 = (int)__reduce_min_sync(0xffffffffu, (uint32_t)first1);
-        const bool gave_up = !tile_wait(Q_READY, pieces & 1, abort_s);   // (everyone is done with the piece before)
+        // (everyone is done with the piece before: this warp may be as far ahead as a whole piece)
+        const bool gave_up = !long_wait(Q_READY, pieces & 1, jobs_done, abort_s);
         if (__any_sync(0xffffffffu, gave_up)) break;
         if (lane == 0) {
           *odd_s = make_int2(first0, first1);
@@ -846,7 +867,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         }
       };
       const float m = lim != PA_MOST_LOG2 ? PA_NOTHING : f == f0 ? ref : ref * (f0 / f);   // (of exponents by f0)
-      if (!wait_for(ODD_READY, (pieces - 1) & 1)) break;
+      {
+        const bool gave_up = !long_wait(ODD_READY, (pieces - 1) & 1, looked_at, abort_s);
+        bad = __any_sync(0xffffffffu, gave_up);
+        if (bad) break;
+      }
       const int odd_0 = odd_s->x, odd_1 = odd_s->y;
       if (two) {
         const bool live = r < rows;
