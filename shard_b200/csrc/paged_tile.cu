@@ -202,7 +202,9 @@ __device__ __forceinline__ void tile_unpack(unsigned char* tile, int row, const 
 
 // A bounded wait as mbar_wait is (tens of milliseconds at least), without a time to sleep: with one, the warps that wait
 // issue three quarters of all instructions, most of them between two naps.
+// (HEED: someone else giving up ends it too)
 constexpr int PT_WAIT_TRIES = 1 << 20;
+template <bool HEED = true>
 __device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   for (int i = 0; i < PT_WAIT_TRIES; ++i) {
     uint32_t ok;
@@ -212,7 +214,7 @@ __device__ __forceinline__ bool tile_wait(uint32_t bar, uint32_t parity, volatil
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     if (ok) return true;
-    if ((i & 63) == 63 && *abort_flag) break;
+    if (HEED && (i & 63) == 63 && *abort_flag) break;
   }
   *abort_flag = 1;
   return false;
@@ -447,9 +449,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         jobs_a += (uint32_t)(n_jobs + 1) / 2;
         jobs_b += (uint32_t)n_jobs / 2;
       }
-      // whoever gave up: do not leave before the tensor core is done with this CTA's memory
+      // whoever gave up: do not leave before the tensor core is done with this CTA's memory (for as long as a product can take)
       commit(DRAINED);
-      tile_wait(DRAINED, 0, abort_s);
+      tile_wait<false>(DRAINED, 0, abort_s);
     } else if (warp == PT_MMA_WARP + 1) {
       // Values that are no numbers, which the unpacking warps leave out: the first token of each half.
       for (uint32_t pieces = 0; next_piece(); ++pieces) {
