@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
 
     // ---- query: column `g` of the tile, and what the lane's two score columns need to know
     uint32_t q[16], qsum;                                // (qsum: part j of -sum(q) of both halves)
-    float f[2];                                          // factor to the exponent of 2
+    float f0[2], f[2];                                   // what a score is times for the exponent of 2
     int vis[2], vis_min;
     {
       const int col = COLS == 4 ? g & 3 : g, cc = col0 + col, tok = p.over_ratio(cc), head = kv * p.ratio + cc - tok * p.ratio;
@@ -223,9 +223,9 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // largest channel to 2^9 .. 2^10; a query of zeros, or one that is not finite, stays as it is
+      // largest channel to 2^9 .. 2^10, with the sign of `scale`; a query of zeros, or one that is not finite, stays as it is
       const int ex = (int)(__float_as_uint(top) >> 23), up = top == 0.f || ex == 255 ? 127 : min(263 - ex, 250);
-      const float by = __uint_as_float((uint32_t)up << 23), back = __uint_as_float((uint32_t)(254 - up) << 23);
+      const float by = p.scale == 0.f ? 0.f : copysignf(__uint_as_float((uint32_t)up << 23), p.scale), back = __uint_as_float((uint32_t)(254 - up) << 23);
       float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -263,13 +263,13 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
         }
         qsum = as_u32(__halves2half2(part[0], part[1]));
       }
-      // (held at fp32's largest: of bf16 queries from 2^120 on the weights are 0 and 1 all the same)
-      const float factor = fminf(fmaxf(back * (262144.f * p.scale * LOG2E), -3e38f), 3e38f);
+      // (held: of bf16 queries from 2^120 on the weights are 0 and 1 all the same)
+      const float factor = p.scale == 0.f ? 1.f : fminf(fmaxf(back * (262144.f * fabsf(p.scale) * LOG2E), 1e-37f), PA_MOST_F);
       const int see = col < cols ? min(max(seq.pos0 + tok + 1, 0), room) : room;   // (columns without a row hide nothing)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int from = 4 * (2 * j + c);
-        f[c] = __shfl_sync(0xffffffffu, factor, from);
+        f0[c] = f[c] = __shfl_sync(0xffffffffu, factor, from);
         vis[c] = __shfl_sync(0xffffffffu, see, from);
       }
       vis_min = (int)__reduce_min_sync(0xffffffffu, (uint32_t)see);
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
       next = look_up(first + 2 * step);
       const uint32_t off = slot * (PA_GROUP * PG_BYTES);
 
-      // scores of rows g, g + 8 (tokens) and columns 2 j, 2 j + 1, as distances from the reference point
+      // scores of rows g, g + 8 (tokens) and columns 2 j, 2 j + 1
       float s[PA_GROUP][4];
 #pragma unroll
       for (int i = 0; i < PA_GROUP; ++i) {
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
         const float2 s0 = __half22float2(as_half2(kp0 & 0xfff0fff0u)), s1 = __half22float2(as_half2(kp1 & 0xfff0fff0u));
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          s[i][k] = fmaf(fmaf(k < 2 ? s0.y : s1.y, half[1][k], (k < 2 ? s0.x : s1.x) * half[0][k]), f[k & 1], -ref[k & 1]);
+          s[i][k] = fmaf(k < 2 ? s0.y : s1.y, half[1][k], (k < 2 ? s0.x : s1.x) * half[0][k]);
       }
       const int t0 = first * PG_BLOCK;
       const int blocks = FULL ? PA_GROUP : group;
@@ -335,27 +335,22 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
         if (lane < group && !((here >> lane) & 1) && first + lane < blk1 && t0 + PG_BLOCK * lane < room && p.status)
           atomicOr(p.status, PG_BAD_PAGE);
       }
-      float top[2] = {fmaxf(s[0][0], s[0][2]), fmaxf(s[0][1], s[0][3])};
+      float most[2] = {fmaxf(s[0][0], s[0][2]), fmaxf(s[0][1], s[0][3])};
 #pragma unroll
       for (int i = 1; i < PA_GROUP; ++i) {
-        top[0] = fmaxf(top[0], fmaxf(s[i][0], s[i][2]));
-        top[1] = fmaxf(top[1], fmaxf(s[i][1], s[i][3]));
+        most[0] = fmaxf(most[0], fmaxf(s[i][0], s[i][2]));
+        most[1] = fmaxf(most[1], fmaxf(s[i][1], s[i][3]));
       }
-      if (__any_sync(0xffffffffu, top[0] > lim[0] || top[1] > lim[1])) {
+      if (__any_sync(0xffffffffu, fmaf(most[0], f[0], -ref[0]) > lim[0] || fmaf(most[1], f[1], -ref[1]) > lim[1])) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], d));
-          if (top[c] > lim[c]) {                         // (the same for all lanes of a column)
-            const float by = top[c] - PA_HEAD_LOG2, alpha = lim[c] == PA_MOST_LOG2 ? ex2(-by) : 0.f;
-            ref[c] += by;
+          for (int d = 4; d < 32; d <<= 1) most[c] = fmaxf(most[c], __shfl_xor_sync(0xffffffffu, most[c], d));
+          if (fmaf(most[c], f[c], -ref[c]) > lim[c]) {   // (the same for all lanes of a column)
+            float alpha = pa_move(most[c], f0[c], f[c], ref[c]);
+            if (lim[c] != PA_MOST_LOG2) alpha = 0.f;
             lim[c] = PA_MOST_LOG2;
             l[c] *= alpha;
-#pragma unroll
-            for (int i = 0; i < PA_GROUP; ++i) {
-              s[i][c] -= by;
-              s[i][2 + c] -= by;
-            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               o[i][c] *= alpha;
@@ -371,7 +366,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
         const uint32_t o_ = off + i * PG_BYTES;
         float w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = ex2(s[i][k]);
+        for (int k = 0; k < 4; ++k) w[k] = ex2(fmaf(s[i][k], f[k & 1], -ref[k & 1]));
         l[0] += w[0] + w[2];
         l[1] += w[1] + w[3];
         // weights as two fp16 parts, transposed: tokens 2 j, 2 j + 1 (and 8 on) of column g
@@ -444,7 +439,12 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
     const int hold = PA_HOLD * step, first_hold = first + hold;
     auto add_held = [&]() {
       const float4 at = held[8 * 32];
-      const float by[2] = {ex2(at.x - ref[0]), ex2(at.y - ref[1])};
+      float m[2], by[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float scale = pa_record(ref[c], f[c], f0[c], m[c]);
+        by[c] = ex2((c ? at.y : at.x) - m[c]) / scale;
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float4 h = held[i * 32];
@@ -459,12 +459,15 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
       if (first == next_hold) {
         if (first != first_hold) add_held();
         next_hold += hold;
+        float m[2], by[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) by[c] = pa_record(ref[c], f[c], f0[c], m[c]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          held[i * 32] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+          held[i * 32] = make_float4(o[i][0] * by[0], o[i][1] * by[1], o[i][2] * by[0], o[i][3] * by[1]);
           o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         }
-        held[8 * 32] = make_float4(lim[0] == PA_MOST_LOG2 ? ref[0] : PA_NOTHING, lim[1] == PA_MOST_LOG2 ? ref[1] : PA_NOTHING, 0.f, 0.f);
+        held[8 * 32] = make_float4(lim[0] == PA_MOST_LOG2 ? m[0] : PA_NOTHING, lim[1] == PA_MOST_LOG2 ? m[1] : PA_NOTHING, 0.f, 0.f);
       }
       if (group == PA_GROUP) turn(std::true_type());
       else turn(std::false_type());
@@ -488,13 +491,15 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float* rec = state(warp, 2 * j + c);
-        if (g == 0) *reinterpret_cast<float2*>(rec) = make_float2(lim[c] == PA_MOST_LOG2 ? ref[c] : PA_NOTHING, l[c]);
+        float m;
+        const float by = pa_record(ref[c], f[c], f0[c], m);
+        if (g == 0) *reinterpret_cast<float2*>(rec) = make_float2(lim[c] == PA_MOST_LOG2 ? m : PA_NOTHING, l[c] * by);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const float (&e0)[4] = o[4 * h + 2 * u], (&e1)[4] = o[4 * h + 2 * u + 1];
-            *reinterpret_cast<float4*>(rec + 4 + 64 * h + 8 * g + 4 * u) = make_float4(e0[c], e0[2 + c], e1[c], e1[2 + c]);
+            *reinterpret_cast<float4*>(rec + 4 + 64 * h + 8 * g + 4 * u) = make_float4(e0[c] * by, e0[2 + c] * by, e1[c] * by, e1[2 + c] * by);
           }
       }
     }

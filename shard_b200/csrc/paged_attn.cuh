@@ -19,6 +19,12 @@ constexpr int PA_SHORT_ROWS = 24;
 // a weight would pass 2^15: the two fp16 parts of a weight reach down to 2^-32 of the largest that way.
 constexpr float PA_HEAD_LOG2 = 7.f, PA_MOST_LOG2 = 15.f;
 constexpr float PA_NOTHING = -3e38f;                     // reference point before the first visible token
+// A weight is 2 to the power of score * f - reference point, one fused operation, and what is scaled from one reference
+// point to another is scaled by the difference of these very numbers: equal keys have equal weights, in whichever block,
+// warp or piece they lie.  From 2^28 on no fp32 number is near enough to every product.  There different scores are 16 apart
+// at least (as exponents), so a factor that makes them more changes nothing: f becomes the next power of two, and the
+// product with the largest score is a number.
+constexpr float PA_FAR = 268435456.f, PA_MOST_F = 8.5e37f;    // (2^126: the next power of two is one too)
 
 // The tensor core cuts off what an fp32 accumulator has no bits for: some 2^-24 of a sum is lost with every product of 16
 // tokens, always toward zero (131 072 tokens in one accumulator: 7e-4, more than an fp16 output's rounding).  So both
@@ -54,6 +60,25 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+__device__ __forceinline__ float one_over(float power_of_two) { return __uint_as_float(0x7f000000u - __float_as_uint(power_of_two)); }
+// The reference point moves to a largest score `most`: f and ref are the new ones (f0 the true f), the result is what sums
+// so far have to be scaled by.
+__device__ __forceinline__ float pa_move(float most, float f0, float& f, float& ref) {
+  const float was = ref, was_f = f, near = fmaf(most, f0, -PA_HEAD_LOG2);
+  f = fabsf(near) < PA_FAR ? f0 : __uint_as_float((__float_as_uint(f0) + 0x7fffffu) & 0x7f800000u);
+  ref = fabsf(near) < PA_FAR ? near : most * f;
+  return ex2(was_f == f ? was - ref : was_f == f0 ? -fmaf(most, f0, -was) : fmaf(was * one_over(was_f), f0, -ref));
+}
+// The reference point as others are to see it, of products with f0: a number m, and what sums have to be scaled by for it (1
+// unless f is not f0; the rest of the largest product, while 2 to its power is a number of a sensible size).
+__device__ __forceinline__ float pa_record(float ref, float f, float f0, float& m) {
+  m = ref;
+  if (f == f0) return 1.f;
+  const float most = ref * one_over(f);
+  m = most * f0;
+  return fabsf(m) < 4.f * PA_FAR ? ex2(fmaf(most, f0, -m)) : 1.f;
 }
 
 // 1024 + the nibbles that `mask` leaves (16 times them from bits 4-7), in both halves

@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             const int ex = (int)(__float_as_uint(top) >> 23), up = top == 0.f || ex == 255 ? 127 : min(263 - ex, 250);
             const float back = __uint_as_float((uint32_t)(254 - up) << 23);
             const float by = p.scale == 0.f ? 0.f : copysignf(__uint_as_float((uint32_t)up << 23), p.scale);
-            if (c == 0) f_s[at[i]] = p.scale == 0.f ? 1.f : fmaxf(back * mag, 1e-37f);
+            if (c == 0) f_s[at[i]] = p.scale == 0.f ? 1.f : fminf(fmaxf(back * mag, 1e-37f), PA_MOST_F);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] *= by;
             const uint4 v = make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1], x[5]), pack_half2(x[2], x[6]), pack_half2(x[3], x[7]));
@@ -656,8 +656,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
       __syncwarp();
       if (lane == 0) mbar_arrive(Q_READY);
       if (!wait_for(Q_READY, pieces++ & 1)) break;
-      const float f0 = f_s[r];                           // factor to the exponent of 2
-      float f = f0;
+      float f = f_s[r];                                  // what a score is times for the exponent of 2
 
       float ref = 0.f, lim = PA_NOTHING, l = 0.f;
       const int32_t* table = p.c.page_table + walk.b * p.c.table_stride;
@@ -669,15 +668,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
       bool missing = t_first < k1 && page_missing(t_first);
       bool fresh = true;                                 // no product in the accumulator yet
       // (a run has at most two pieces of units that others share: its first piece, and its last)
-      float* records = p.part + (2 * (int64_t)blockIdx.x + (first_piece ? 0 : 1)) * PT_ROWS * PART;
+      auto records = [&]() { return p.part + (2 * (int64_t)blockIdx.x + (first_piece ? 0 : 1)) * PT_ROWS * PART; };
       // What the accumulator had before its last PT_HOLD tiles waits where the piece's result will go, four channels of
       // all lanes side by side: held = held * by + accumulator * scale.
-      float held_ref = PA_NOTHING;                       // its reference point
-      float4* held = reinterpret_cast<float4*>(records + (warp * 32) * PART) + lane;
+      auto held = [&]() { return reinterpret_cast<float4*>(records() + (warp * 32) * PART) + lane; };
+      auto held_by = [&]() {                             // (its reference point is behind it)
+        float m;
+        const float scale = pa_record(ref, f, f_s[r], m);
+        return ex2(held()[32 * 32].x - m) / scale;
+      };
       auto add_held = [&](uint32_t (&o)[16], int c, float scale, float by, bool has) {   // channels 16 c ..
         float4 h[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = has ? held[(4 * c + i) * 32] : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < 4; ++i) h[i] = has ? held()[(4 * c + i) * 32] : make_float4(0.f, 0.f, 0.f, 0.f);
         tmem_ld_x16(O + 16 * c, o);
         tmem_wait_ld();
 #pragma unroll
@@ -722,19 +725,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             if (!((seen >> i) & 1)) s[i] = 0xff800000u;
         };
         auto refer = [&]() {                             // the reference point follows
-          const float most = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), top = fmaf(most, f, -ref);
-          if (top > lim) {
-            const float by = top - PA_HEAD_LOG2;
-            alpha = lim == PA_MOST_LOG2 ? ex2(-by) : 0.f;
-            ref += by;
+          const float most = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          if (fmaf(most, f, -ref) > lim) {
+            alpha = pa_move(most, f_s[r], f, ref);
+            if (lim != PA_MOST_LOG2) alpha = 0.f;
             lim = PA_MOST_LOG2;
-            // An exponent is the exact product less a rounded reference point, which from 2^28 on may be more than 2^8 away.
-            // There different scores are 32 apart at least: a factor that makes them more changes nothing, and with a power
-            // of two the product is a number.
-            if (fabsf(ref) >= 268435456.f) {
-              f = __uint_as_float((__float_as_uint(f) + 0x7fffffu) & 0x7f800000u);
-              ref = most * f;
-            }
           }
         };
         auto weigh = [&](const uint32_t (&s)[32], int c) {   // weights in the place of the scores
@@ -796,16 +791,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         // (the group's product before this one has run: the scores were issued behind it)
         const int nth = (tile - t_first) >> (two ? 0 : 1);   // of the group's tiles of the piece
         if (nth % PT_HOLD == 0 && nth > 0) {             // the product to come begins the accumulator anew
-          const float by = ex2(held_ref - ref);
+          float m;
+          const float scale = pa_record(ref, f, f_s[r], m), by = nth > PT_HOLD ? ex2(held()[32 * 32].x - m) : 0.f;
 #pragma unroll 4
           for (int c = 0; c < 8; ++c) {
             uint32_t o[16];
-            add_held(o, c, alpha, by, nth > PT_HOLD);
+            add_held(o, c, alpha * scale, by, nth > PT_HOLD);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) held[(4 * c + i) * 32] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+            for (int i = 0; i < 4; ++i) held()[(4 * c + i) * 32] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
                                                                             __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
           }
-          held_ref = lim == PA_MOST_LOG2 ? ref : PA_NOTHING;
+          held()[32 * 32] = make_float4(lim == PA_MOST_LOG2 ? m : PA_NOTHING, 0.f, 0.f, 0.f);
         } else if (!fresh && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
           for (int c = 0; c < 8; ++c) {
@@ -829,7 +825,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
       // ---- the piece's result
       const bool finish = walk.whole;
       if (k1 - t_first > PT_HOLD * stride && warp_live) {                  // (the records that may lie there are written once all warps have read)
-        const float by = ex2(held_ref - ref);
+        const float by = held_by();
 #pragma unroll 4
         for (int c = 0; c < 8; ++c) {
           uint32_t o[16];
@@ -854,13 +850,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         return finish ? (int64_t)(walk.seq_first + tok) * p.n_q + walk.kv * p.ratio + cc - tok * p.ratio : (int64_t)of_unit;
       };
       auto put_sums = [&](int64_t at, float m, float sum) {
-        if (!finish) *reinterpret_cast<float2*>(records + at * PART) = make_float2(m, sum);
+        if (!finish) *reinterpret_cast<float2*>(records() + at * PART) = make_float2(m, sum);
         else if (p.lse) p.lse[at] = sum == 0.f ? neg_inf() : (m + log2f(sum)) * LN2;
       };
       // eight channels from 8 c on of a row; the products leave them in the order 0 4 1 5 2 6 3 7
       auto put8 = [&](int64_t at, int c, const float (&x)[8]) {
         if (!finish) {
-          float4* dst = reinterpret_cast<float4*>(records + at * PART + 4 + 8 * c);
+          float4* dst = reinterpret_cast<float4*>(records() + at * PART + 4 + 8 * c);
           dst[0] = make_float4(x[0], x[2], x[4], x[6]);
           dst[1] = make_float4(x[1], x[3], x[5], x[7]);
         } else {
@@ -868,7 +864,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
               make_uint4(Pair<T>::put(x[0], x[2]), Pair<T>::put(x[4], x[6]), Pair<T>::put(x[1], x[3]), Pair<T>::put(x[5], x[7]));
         }
       };
-      const float m = lim != PA_MOST_LOG2 ? PA_NOTHING : f == f0 ? ref : ref * (f0 / f);   // (of exponents by f0)
+      float m;
+      const float scale = pa_record(ref, f, f_s[r], m);
+      if (lim != PA_MOST_LOG2) m = PA_NOTHING;
+      l *= scale;
       {
         const bool gave_up = !long_wait(ODD_READY, (pieces - 1) & 1, looked_at, abort_s);
         bad = __any_sync(0xffffffffu, gave_up);
@@ -877,7 +876,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
       const int odd_0 = odd_s->x, odd_1 = odd_s->y;
       if (two) {
         const bool live = r < rows;
-        const float inv = !finish ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        const float inv = !finish ? scale : l == 0.f ? 0.f : scale / l;
         const int64_t at = row_of(r);
         if (live) put_sums(at, m, l);
 #pragma unroll 1
@@ -913,7 +912,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
               tmem_wait_ld();
               float* to = join_s + (state * 64 + 32 * c) * copy_rows + row % copy_rows;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) to[e * copy_rows] = __uint_as_float(o[e]);
+              for (int e = 0; e < 32; ++e) to[e * copy_rows] = __uint_as_float(o[e]) * scale;
             }
           }
           __syncwarp();
