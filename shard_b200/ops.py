@@ -546,7 +546,7 @@ def paged_attn(q, pool, page_table, cu, lens, scale=None, max_new=None, out=None
     more new tokens than this (None: not known; a value picks the kernels that such a call needs).  lse
     (rows, n_q) fp32: receives the logarithm of each row's sum of weights.  A row that sees no token is zero."""
     scale = HD ** -0.5 if scale is None else float(scale)
-    if pool.is_cuda and (done := _paged_native(_lib.host().paged_attn(pool, page_table, cu, lens, q, scale, -1 if max_new is None else max(int(max_new), -2),
+    if pool.is_cuda and (done := _paged_native(_lib.host().paged_attn(pool, page_table, cu, lens, q, scale, -1 if max_new is None else int(max_new) if max_new >= 0 else -2,
                                                                       out, lse, status), "paged_attn")) is not None:
         return done
     cache = _paged(pool, page_table, cu, lens)
