@@ -10,8 +10,9 @@ come, grow and go independently.  It keeps the pages' books on the host; the ari
     cache.begin({a: 700, b: 90})                      # two prompts, one behind the other
     for i, layer in enumerate(layers):                # q (790, n_q, 128), k and v (790, n_kv_heads, 128)
         out = cache.attend(i, q, k, v)
-    cache.begin({a: 1, b: 1})                         # the next token of both
+    cache.begin({a: 1, b: 5})                         # the next token of one, five drafted ones of the other
     ...
+    cache.truncate(b, cache.length(b) - 3)            # of which two were accepted
     cache.remove(a)
 """
 from __future__ import annotations
@@ -70,6 +71,17 @@ class PagedCache:
         """Forgets a sequence; its pages are free for calls that are made from now on."""
         self._free.extend(reversed(self._pages(seq)))
         self._slots[seq], self._lens[seq], self._batch = None, 0, None
+
+    def truncate(self, seq, tokens):
+        """Keeps a sequence's first `tokens` tokens and forgets the others (drafted ones that were not accepted); pages
+        that hold none of the first are free for calls that are made from now on.  begin() comes before the next step."""
+        pages, tokens = self._pages(seq), int(tokens)
+        if not 0 <= tokens <= self._lens[seq]:
+            raise ShardError(f"sequence {seq} has {self._lens[seq]} tokens and cannot keep {tokens}")
+        kept = -(-tokens // self.page_size)
+        self._free.extend(reversed(pages[kept:]))
+        del pages[kept:]
+        self._lens[seq], self._batch = tokens, None
 
     def length(self, seq):
         self._pages(seq)

@@ -253,3 +253,32 @@ def test_rotation_table():
     pos = torch.tensor([0, 1, 5, 77, 1000, 8190, 8191])
     t = rope_table(8192, inv)[pos]
     assert torch.equal(P.rotate(x[:, None], t[:, :64], t[:, 64:])[:, 0], reapply_rope(x, pos, inv))
+
+
+def test_books_of_truncated_sequences():
+    from shard_b200 import PagedCache
+    c = PagedCache(1, 2, 6, 2, 100, torch.ones(64), page_size=16, device="cpu")
+    a, b = c.add(), c.add()
+    c.begin({a: 40, b: 16})
+    first, freed = c._slots[a][:2], c._slots[a][2]
+    for tokens in (41, -1):
+        with pytest.raises(ShardError):
+            c.truncate(a, tokens)
+    assert c.length(a) == 40 and c.free_pages == 2 and c._batch is not None
+    c.truncate(a, 33)                          # the third page still holds a token
+    assert c.length(a) == 33 and c.free_pages == 2 and c._slots[a] == first + [freed]
+    with pytest.raises(ShardError):
+        c.append(0, torch.zeros(56, 2, 128), torch.zeros(56, 2, 128))      # begin() comes first
+    c.truncate(a, 32)
+    assert c.length(a) == 32 and c.free_pages == 3 and c._slots[a] == first
+    c.begin({b: 1, a: 1})
+    assert c._slots[b][1] == freed and c._batch[2].tolist() == [17, 33] and len({*c._slots[a], *c._slots[b]}) == 5
+    c.truncate(b, 0)
+    assert c.length(b) == 0 and c.free_pages == 3 and c._slots[b] == []
+    c.begin({b: 20})
+    assert c.length(b) == 20 and c.memory_bytes() == 5 * 2 * 2176
+    c.remove(b)
+    c.truncate(a, 33)
+    assert c.length(a) == 33 and c.free_pages == 3
+    with pytest.raises(ShardError):
+        c.truncate(b, 0)
