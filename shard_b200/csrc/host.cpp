@@ -225,7 +225,7 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---- the paged 4-bit cache -----------------------------------------------------------------------
-// One launch each, which take the GPU a few microseconds: the Python forms of these calls take twenty.  What these
+// One to four launches, which take the GPU a few microseconds in small calls: the Python forms of these take twenty.  What these
 // do not take as it is (strides to be copied, a wrong argument) is the Python forms' to do or to refuse.
 using PagedAppendFn = int (*)(const ShardPaged*, const void*, const void*, const void*, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int32_t,
                               int32_t, int32_t, const float*, int32_t, void*, int*, void*);
