@@ -37,7 +37,7 @@ constexpr int PT_UNPACK_WARP = 8, PT_MMA_WARP = 12;
 constexpr int PT_THREADS = 32 * (PT_MMA_WARP + 4);       // (registers change hands by fours of warps)
 // Registers of a thread, whose sum over the four fours of warps is what the block is launched with (128 each).  A row's
 // 128 scores are to stay in registers: reading them from tensor memory a second time takes 200 cycles for every 32.
-constexpr int PT_REGS_SOFTMAX = 184, PT_REGS_UNPACK = 104, PT_REGS_MMA = 40;
+constexpr int PT_REGS_SOFTMAX = 200, PT_REGS_UNPACK = 80, PT_REGS_MMA = 32;
 static_assert(2 * PT_REGS_SOFTMAX + PT_REGS_UNPACK + PT_REGS_MMA == 4 * 128, "no more than the block was launched with");
 constexpr int PT_ROWS = 256;                             // of a unit
 constexpr int PT_KEYS = 128;                             // of a tile
@@ -234,6 +234,19 @@ __device__ __forceinline__ bool long_wait(uint32_t bar, uint32_t parity, const v
   }
   *abort_flag = 1;
   return false;
+}
+// two fp32 operations in an instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
 // single-thread forms of the products (the caller is one thread)
 __device__ __forceinline__ void product_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
@@ -702,7 +715,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
         }
         const int limit = vis - PT_KEYS * tile;
         const bool edge = __any_sync(0xffffffffu, limit < PT_KEYS) || holes;
-        float mx[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()}, alpha = 1.f, sum[2] = {0.f, 0.f};
+        float mx[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()}, alpha = 1.f;
+        float2 sum = make_float2(0.f, 0.f);
         const int c0 = copy * (4 / copies), c1 = c0 + 4 / copies;     // its quarters of the tile's keys
         if (copies > 1) {                                // no weights for the other copies' keys
           uint32_t zero[16];
@@ -736,12 +750,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float a = ex2(fmaf(__uint_as_float(s[2 * i]), f, -ref)), d = ex2(fmaf(__uint_as_float(s[2 * i + 1]), f, -ref));
-            sum[0] += a;
-            sum[1] += d;
-            hi[i] = pack_half2(a, d);
-            const float2 rest = __half22float2(as_half2(hi[i]));
-            lo[i] = pack_half2(a - rest.x, d - rest.y);
+            const float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), make_float2(f, f), make_float2(-ref, -ref));
+            const float2 w = make_float2(ex2(x.x), ex2(x.y));
+            sum = add2(sum, w);
+            hi[i] = pack_half2(w.x, w.y);
+            const float2 rest = fma2(__half22float2(as_half2(hi[i])), make_float2(-1.f, -1.f), w);
+            lo[i] = pack_half2(rest.x, rest.y);
           }
           tmem_st_x16(S + 32 * c, hi);
           tmem_st_x16(S + 32 * c + 16, lo);
@@ -787,7 +801,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tile_kernel(const __grid_
             weigh(s, c);
           }
         }
-        l = l * alpha + (sum[0] + sum[1]);
+        l = l * alpha + (sum.x + sum.y);
         // (the group's product before this one has run: the scores were issued behind it)
         const int nth = (tile - t_first) >> (two ? 0 : 1);   // of the group's tiles of the piece
         if (nth % PT_HOLD == 0 && nth > 0) {             // the product to come begins the accumulator anew
