@@ -18,10 +18,10 @@
 //            (1024 + code) - (1024 + z) and the product with the scale are exact in fp16.  A weight is two fp16 parts
 //            (22 bits, see PA_HEAD_LOG2): up to four rows fill a tile's eight columns with them, so that they are free there.
 //
-// What bounds it: instructions.  A block is some 366 of a warp's (half of them masks, shifts and fp16 arithmetic that
+// What bounds it: instructions.  A block is some 375 of a warp's (half of them masks, shifts and fp16 arithmetic that
 // unpack) and takes a scheduler 600 cycles with three warps to choose from; the bytes would come 1.7 times as fast.  64
-// sequences of up to 8 192 tokens, 8 KV heads, 4 query heads to each (433 MB): 113 to 117 us, 3.8 TB/s; one of 131 072 (143 MB):
-// 44 us, 3.3 TB/s.  Fixed part of a launch, some 10 000 cycles: adding the list up 2 000, the query 2 000, the first
+// sequences of up to 8 192 tokens, 8 KV heads, 4 query heads to each (433 MB): 117 us, 3.7 TB/s; one of 131 072 (143 MB):
+// 45 us, 3.2 TB/s.  Fixed part of a launch, some 10 000 cycles: adding the list up 2 000, the query 2 000, the first
 // blocks 1 300, joining the warps; then the launch that joins the CTAs, 3 to 5 us.
 #include <atomic>
 #include <type_traits>
@@ -88,7 +88,7 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 
 // COLS: query rows to a tile.  4: the tile's other four columns carry the same rows again, and then the low parts of
 // their weights.  8: two products for the two parts.  Chosen by a sequence's largest number of rows: four rows in eight
-// columns take 120 us where four take 113 (64 sequences of up to 8 192 tokens, 8 KV heads), eight rows 121 and 213.
+// columns take 157 us where four take 147 (64 sequences of 8 192 tokens, 8 KV heads), eight rows 158 and 278.
 template <typename T, int COLS>
 __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(const __grid_constant__ PagedAttnParams p) {
   extern __shared__ __align__(16) unsigned char pa_smem[];
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(32 * PA_WARPS, PA_CTAS) paged_split_kernel(con
 
 // Joins the pieces of the work that begins in a CTA's run and ends behind it, always in the same order.  A CTA looks
 // after PM_RUNS runs: work in up to PM_DEPTH pieces takes a warp a row, all of them in flight at once; work in more,
-// as of one long sequence, takes all warps.
+// as of one long sequence, takes all warps.  (With 8 columns a block has 1 024 threads of 64 registers, and 36 bytes spill.)
 constexpr int PM_RUNS = 4, PM_DEPTH = 8;
 template <typename T, int COLS>
 __global__ void __launch_bounds__(32 * COLS * PM_RUNS) paged_merge_kernel(const __grid_constant__ PagedAttnParams p, int runs) {

@@ -10,9 +10,11 @@
 namespace shard {
 
 // Sequences with more query rows to a KV head (new tokens times query heads of it) are paged_tile.cu's; the others too
-// where, going by the sizes, all have more: paged_attn.cu's launches would find nothing to do.  64 sequences of up to
-// 8 192 tokens, 8 KV heads, paged_attn.cu / paged_tile.cu: 16 rows 230 / 397 us, 24 rows 337 / 397, 32 rows 446 / 397
-// (which cost the tiles the same, in four copies).  One of 2 051 tokens: 32 rows 14 / 26 us.
+// where, going by the sizes, all have more: paged_attn.cu's launches would find nothing to do.  64 sequences of 8 192
+// tokens, 8 KV heads, paged_attn.cu / paged_tile.cu: 16 rows 298 / 513 us, 24 rows 439 / 514, 32 rows 620 / 535 (which cost
+// the tiles the same, in four copies).  Up to 24 rows paged_attn.cu was faster at every length and number of sequences
+// measured.  Of short sequences it is with more, too, so that rows alone put the border too low for them: 32 rows of 64
+// sequences of 2 051 tokens 170 / 210 us, of one 15 / 26; 48 rows of one 16 / 27, of 64 247 / 220.
 constexpr int PA_SHORT_ROWS = 24;
 
 // A row's reference point is put PA_HEAD below its largest score so far, which then has the weight 2^7, and stays until

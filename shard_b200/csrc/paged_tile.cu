@@ -19,12 +19,13 @@
 //
 // The eight channels of a 32-bit word are unpacked in the order 0 4 1 5 2 6 3 7, in which two nibbles at a time leave
 // it; queries are staged in that order, and the output is put back.  Weights are two fp16 parts (22 bits, as in
-// paged_attn.cu), each product run twice: the first part alone (bf16 outputs, 415 us) moves one output in twenty by a
-// last place.
+// paged_attn.cu), each product run twice: with the first part alone bf16 outputs would take two thirds of the time, and
+// one in twenty would be a last place off.
 //
-// What bounds it: the chain of a step, 4 370 cycles a job: products with the weights, their end, scores, and the
-// softmax of 128 numbers a thread, which the other group's products hide only in part.  2 048 rows x 4 query heads
-// behind 8 192 tokens, 8 KV heads (309 GFLOP): 675 us, 458 TFLOP/s, bf16 and fp16 alike.  Start
+// What bounds it: the chain of a step, 4 200 cycles a job: products with the weights, their end, scores, and the
+// softmax of 128 numbers a thread, which the other group's products hide only in part and whose straight line of
+// instructions is more than their cache holds (after tensor memory, the longest waits are for those).  2 048 rows x 4 query
+// heads behind 8 192 tokens, 8 KV heads (309 GFLOP): 650 us, 475 TFLOP/s, bf16 and fp16 alike.  Start
 // and result of a piece are some 8 000 cycles each.  Measured and slower: a thread for each group's products (470 us),
 // eight unpacking warps with the scores read from tensor memory twice (485 us).
 #include <atomic>
