@@ -14,10 +14,11 @@ namespace shard {
 //   s = fp16((max(x, 0) - min(x, 0)) * (1 / 15)) rounded to 7 significant bits (1 / 15 as an fp32 number),  z = rint(-min / s),
 //   code = rint(x / s) + z, within 0 .. 15        (quotients, since 16-bit inputs do lie on the borders of codes)
 //
-// What bounds it: a warp's some 500 instructions and, in small calls, its chain of loads (tables, then angles).  8 191
-// tokens of 8 KV and 32 query heads, bf16 (101 MB in, 77 MB out): 40 us, 4.5 TB/s; 64 tokens: 5.6 us.  A warp takes eight
-// vectors of a token rather than one vector: a maximum over 64 channels is two exchanges, not five, and angles are
-// loaded once for the eight.
+// What bounds it: a warp waits for its rows, then computes (some 500 instructions) with nothing of its own in flight, and
+// the 40 % of the warps that fit hide only a part of either from the other; in small calls, its chain of loads (tables, then
+// angles).  8 191 tokens of 8 KV and 32 query heads, bf16 (101 MB in, 77 MB out): 40 us, 4.5 TB/s; 64 tokens: 5.6 us.  A
+// warp takes eight vectors of a token rather than one vector: a maximum over 64 channels is two exchanges, not five, and
+// angles are loaded once for the eight.
 struct PagedAppendParams {
   ShardPaged c;
   const void *k, *v, *q;
