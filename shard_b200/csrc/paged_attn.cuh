@@ -40,7 +40,7 @@ struct PagedAttnParams {
   void* out;                                             // [rows][n_q][128]
   float* lse;                                            // [rows][n_q] or null
   int* status;
-  float* part;                                           // [2 grid][cols][132]
+  float* part;                                           // [2 grid][cols][132], and the split kernel's accumulators that are put aside
   int4* items;                                           // [grid] of the work that begins in a CTA's run and ends behind it
   float scale;
   int n_q, rows, max_new, ratio;
